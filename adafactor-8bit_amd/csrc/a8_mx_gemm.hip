@@ -2,6 +2,7 @@
 // a [m, k] and b [n, k] as MX tensors (a8_mx.cuh), fp32 accumulation in the matrix cores.
 #include "a8_abi_impl.h"
 #include "a8_mx.cuh"
+#include "a8_mx_lds.h"
 
 namespace a8 {
 namespace {
@@ -408,28 +409,31 @@ __global__ __launch_bounds__(256 * KG, MI * NI == 16 || KG > 1 ? 1 : 2) void k_m
   // A lane (r, h) holds of a 32 x 32 tile row r, columns 8 q + 4 h + (0..3).  Through LDS (a part of
   // it for each wave) 32 rows become runs of 16 bytes a lane, whole rows of the wave's columns.
   mx_wait_barrier<0>();
+  typedef MxEnd<NI, KG, (int)sizeof(T)> End;
+  static_assert(End::kBytes <= Stage::kLds, "");
   if constexpr (KG > 1) {
-    static_assert(MI == 1 && NI == 1 && KG * 4 * 4096 <= Stage::kLds, "");
+    static_assert(MI == 1 && NI == 1, "");
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-    lds_f32x4* sums = (lds_f32x4*)((lds_u8*)smem) + wave * 256 + lane;   // [group][wave][quarter][lane]
+    lds_u8* sums = (lds_u8*)smem + lane * 16;   // of a wave: a quarter of its sums for each lane, then the next
     if (group)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        sums[group * 1024 + e * 16] = f32x4{acc[0][0][e], acc[0][0][e + 1], acc[0][0][e + 2], acc[0][0][e + 3]};
+        *(lds_f32x4*)(sums + End::sums(group, wave) + e * 256) =
+            f32x4{acc[0][0][e], acc[0][0][e + 1], acc[0][0][e + 2], acc[0][0][e + 3]};
     mx_wait_barrier<0>();
     if (group) return;
 #pragma unroll
     for (int g = 1; g < KG; ++g)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const f32x4 t = sums[g * 1024 + e * 16];
+        const f32x4 t = *(lds_f32x4*)(sums + End::sums(g, wave) + e * 256);
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[0][0][e + j] += t[j];
       }
   }
-  constexpr int kCols = 32 * NI, kOut = kCols * (int)sizeof(T) + 16, kPart = 32 * kOut;
+  constexpr int kCols = 32 * NI, kOut = End::kRow;
   constexpr int V = 16 / (int)sizeof(T), kLanes = kCols / V;   // elements a lane, lanes a row
-  lds_u8* mine = lds + wave * kPart;
+  lds_u8* mine = lds + End::staged(wave);   // group 0's part of the LDS starts where all of it does
 #pragma unroll
   for (int f = 0; f < MI; ++f) {
 #pragma unroll
