@@ -41,8 +41,9 @@ class MXTensor:
     ``scales``: uint8 [rows, P / 32], byte b for 2^(b - 127) and 255 for NaN; P is ``cols`` rounded
     up to 256, and the codes beyond ``cols`` are 0.  Both on the GPU, contiguous, 16-byte aligned.
     """
-    # cp, sp: addresses of the codes and scales; keep: the tensors that hold them; f: the format's number
-    __slots__ = ("rows", "cols", "fmt", "f", "device", "cp", "sp", "keep")
+    # keep: the codes and the scales, or the one buffer that holds both; f: the format's number.  Addresses are
+    # read from `keep` for every call: a copy of the object, or parts whose memory was replaced, have others
+    __slots__ = ("rows", "cols", "fmt", "f", "keep")
 
     def __init__(self, codes, scales, cols, fmt):
         f = _code(_FMT, fmt, "fmt")
@@ -55,11 +56,22 @@ class MXTensor:
             raise TypeError("adafactor8bit: codes and scales of an MX tensor are uint8")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("adafactor8bit: codes and scales of an MX tensor are contiguous")
-        self.device = codes.device
-        if self.device != scales.device:
+        if codes.device != scales.device:
             raise ValueError("adafactor8bit: codes and scales of an MX tensor are on one device")
-        self.rows, self.cols, self.fmt, self.f = rows, cols, fmt, f
-        self.cp, self.sp, self.keep = codes.data_ptr(), scales.data_ptr(), (codes, scales)
+        self.rows, self.cols, self.fmt, self.f, self.keep = rows, cols, fmt, f, (codes, scales)
+
+    def __reduce__(self):   # copies and pickles are made of the parts
+        return MXTensor, (self.codes, self.scales, self.cols, self.fmt)
+
+    def _addresses(self):
+        """Of the codes and the scales, and the number of the GPU that they are on (-1: none)."""
+        keep = self.keep
+        codes = keep[0]
+        at = codes.data_ptr()
+        if len(keep) == 1:
+            return at, at + self.rows * ((self.cols + 255 & -256) >> (1 - self.f)), codes.get_device()
+        i = codes.get_device()
+        return at, keep[1].data_ptr(), i if keep[1].get_device() == i else -1
 
     def _split(self):
         if len(self.keep) == 1:   # one buffer from _over: the codes, then the scales
@@ -78,6 +90,10 @@ class MXTensor:
         return self._split()[1]
 
     @property
+    def device(self):
+        return self.keep[0].device
+
+    @property
     def shape(self):
         return torch.Size((self.rows, self.cols))
 
@@ -88,9 +104,7 @@ class MXTensor:
 def _over(buf, rows, cols, fmt, f):
     """An MX tensor over a buffer of _bytes(rows, cols, f) bytes."""
     t = object.__new__(MXTensor)
-    at = buf.data_ptr()
-    t.rows, t.cols, t.fmt, t.f, t.device, t.keep = rows, cols, fmt, f, buf.device, (buf,)
-    t.cp, t.sp = at, at + rows * (_pitch(cols) >> (1 - f))
+    t.rows, t.cols, t.fmt, t.f, t.keep = rows, cols, fmt, f, (buf,)
     return t
 
 
@@ -109,20 +123,18 @@ def _on_gpu(x, what):
         raise RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got a tensor on {x.device}")
 
 
-def _on_gpu_device(device, what):
-    if device.type != "cuda":
-        raise RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got a tensor on {device}")
+def _not_on_gpu(t, what):
+    return RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got an MX tensor on {t.keep[0].device} and {t.keep[-1].device}")
 
 
 _fn = {}
 
 
-def _launch(name, device, *args):
-    """A library call on the device's current stream, with that device current."""
+def _launch(name, i, *args):
+    """A library call on the current stream of GPU i, with that GPU current."""
     fn = _fn.get(name)
     if fn is None:
         fn = _fn[name] = getattr(nat.lib(), name)
-    i = device.index
     if i == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
@@ -149,9 +161,9 @@ def _quantize(x, fmt, f, along, down, rule, seed):
     dev = x.device
     a = _new(rows, cols, fmt, f, dev) if along else None
     d = _new(cols, rows, fmt, f, dev) if down else None
-    _launch("a8_mx_quantize", dev, _DTYPE[x.dtype], f, rule, seed is not None, x.data_ptr(), rows, cols,
-            x.stride(0) if rows > 1 and cols else cols, a.cp if along else None, a.sp if along else None,
-            d.cp if down else None, d.sp if down else None, 0 if seed is None else seed & _MASK64)
+    _launch("a8_mx_quantize", x.get_device(), _DTYPE[x.dtype], f, rule, seed is not None, x.data_ptr(), rows, cols,
+            x.stride(0) if rows > 1 and cols else cols, *(a._addresses()[:2] if along else (None, None)),
+            *(d._addresses()[:2] if down else (None, None)), 0 if seed is None else seed & _MASK64)
     return a, d
 
 
@@ -180,16 +192,24 @@ def mx_dequantize(t, dtype=torch.bfloat16):
     """The values of an MX tensor as a contiguous [rows, cols] matrix."""
     if dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_dequantize writes fp32, bf16 or fp16, got {dtype}")
-    _on_gpu_device(t.device, "mx_dequantize")
+    cp, sp, i = t._addresses()
+    if i < 0:
+        raise _not_on_gpu(t, "mx_dequantize")
     out = t.keep[0].new_empty((t.rows, t.cols), dtype=dtype)
-    _launch("a8_mx_dequantize", t.device, _DTYPE[dtype], t.f, out.data_ptr(), t.cp, t.sp, t.rows, t.cols)
+    _launch("a8_mx_dequantize", i, _DTYPE[dtype], t.f, out.data_ptr(), cp, sp, t.rows, t.cols)
     return out
 
 
-def _matmul(a, b, out_dtype):
-    m, n, k, dev = a.rows, b.rows, a.cols, a.device
+def _matmul(a, b, out_dtype, what):
+    ac, asc, i = a._addresses()
+    bc, bsc, j = b._addresses()
+    if i < 0 or j < 0:
+        raise _not_on_gpu(a if i < 0 else b, what)
+    if i != j:
+        raise ValueError(f"adafactor8bit: {what}'s operands are on one device")
+    m, n = a.rows, b.rows
     c = a.keep[0].new_empty((m, n), dtype=out_dtype)
-    _launch("a8_mx_matmul", dev, a.f, b.f, _DTYPE[out_dtype], a.cp, a.sp, b.cp, b.sp, c.data_ptr(), m, n, k)
+    _launch("a8_mx_matmul", i, a.f, b.f, _DTYPE[out_dtype], ac, asc, bc, bsc, c.data_ptr(), m, n, a.cols)
     return c
 
 
@@ -201,10 +221,7 @@ def mx_matmul(a, b, out_dtype=torch.bfloat16):
     _code(_DTYPE, out_dtype, "out_dtype")
     if b.cols != a.cols:
         raise ValueError(f"adafactor8bit: mx_matmul of {a.cols} and {b.cols} columns")
-    _on_gpu_device(a.device, "mx_matmul")
-    if b.device != a.device:
-        raise ValueError("adafactor8bit: mx_matmul's operands are on one device")
-    return _matmul(a, b, out_dtype)
+    return _matmul(a, b, out_dtype, "mx_matmul")
 
 
 def first_order(name, gradients):
@@ -229,7 +246,7 @@ class _Linear(torch.autograd.Function):
         wa, wd = _quantize(w, weight, fw, True, need_x, rule, None)
         ctx.save_for_backward(xd.keep[0] if need_w else None, wd.keep[0] if need_x else None)
         ctx.rest = fmts, rule, seed, x.dtype, w.dtype, x.shape[1]
-        return _matmul(xa, wa, x.dtype)
+        return _matmul(xa, wa, x.dtype, "mx_linear")
 
     @staticmethod
     def gradients(ctx, dy):
@@ -238,8 +255,8 @@ class _Linear(torch.autograd.Function):
         dy = _rows(dy)
         m, n = dy.shape
         da, dd = _quantize(dy, grad, fg, wd is not None, xd is not None, rule, seed)
-        dx = _matmul(da, _over(wd, k, n, weight, fw), xt) if wd is not None else None
-        dw = _matmul(dd, _over(xd, k, m, act, fa), wt) if xd is not None else None
+        dx = _matmul(da, _over(wd, k, n, weight, fw), xt, "mx_linear") if wd is not None else None
+        dw = _matmul(dd, _over(xd, k, m, act, fa), wt, "mx_linear") if xd is not None else None
         return dx, dw, None, None, None
 
     backward = first_order("mx_linear", gradients)
@@ -274,7 +291,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
         if weight.device != x.device:
             raise ValueError("adafactor8bit: mx_linear's operands are on one device")
         xa, _ = _quantize(_rows(x.detach()), *fmts[0], True, False, rule, None)
-        y = _matmul(xa, weight, x.dtype)
+        y = _matmul(xa, weight, x.dtype, "mx_linear")
     else:
         if weight.dtype not in _DTYPE:
             raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16 weights, got {weight.dtype}")

@@ -21,9 +21,9 @@ def _forward(x, residual, weight, eps, fmt, keep):
     low = h.new_empty((rows, (cols + 7) // 8), dtype=torch.int32) if keep and h is not None and h.element_size() == 2 else None
     rstd = x.new_empty(rows, dtype=torch.float32) if keep else None
     t = _DTYPE[x.dtype]
-    _launch("a8_rms_norm", dev, t, t if h is None else _DTYPE[h.dtype], _DTYPE[weight.dtype], f, x.data_ptr(), x.stride(0),
+    _launch("a8_rms_norm", x.get_device(), t, t if h is None else _DTYPE[h.dtype], _DTYPE[weight.dtype], f, x.data_ptr(), x.stride(0),
             None if h is None else residual.data_ptr(), 0 if h is None else residual.stride(0), weight.data_ptr(),
-            y.data_ptr() if fmt is None else None, None if fmt is None else y.cp, None if fmt is None else y.sp,
+            *((y.data_ptr(), None, None) if fmt is None else (None, *y._addresses()[:2])),
             None if h is None else h.data_ptr(), None if low is None else low.data_ptr(),
             None if rstd is None else rstd.data_ptr(), rows, cols, eps)
     return y, h, low, rstd
@@ -48,7 +48,7 @@ class _RmsNorm(torch.autograd.Function):
         dr = torch.empty_like(h) if ctx.residual and h.dtype != ctx.dtype else None
         dw = torch.empty_like(weight)
         ws = rstd.new_empty(nat.lib().a8_rms_norm_workspace_floats(rows, cols))
-        _launch("a8_rms_norm_backward", h.device, _DTYPE[ctx.dtype], _DTYPE[h.dtype], _DTYPE[weight.dtype], dy.data_ptr(),
+        _launch("a8_rms_norm_backward", h.get_device(), _DTYPE[ctx.dtype], _DTYPE[h.dtype], _DTYPE[weight.dtype], dy.data_ptr(),
                 None if dh is None else dh.data_ptr(), h.data_ptr(),
                 None if low is None else low.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
                 None if dr is None else dr.data_ptr(), dw.data_ptr(), ws.data_ptr(), rows, cols)
