@@ -3,6 +3,7 @@
 #include "a8_abi_impl.h"
 #include "a8_mx.cuh"
 #include "a8_mx_lds.h"
+#include "a8_once.h"
 
 namespace a8 {
 namespace {
@@ -481,9 +482,14 @@ template <int FA, int FB, int MI, int NI, int KG, typename T>
 int tiles(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, T* c, int64_t m, int64_t n,
           int64_t k, hipStream_t st) {
   constexpr int lds = MxStage<FA, FB, MI, NI, KG>::kLds;
-  static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_tile<FA, FB, MI, NI, KG, T>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (ready != hipSuccess) return set_error(A8_ERR_HIP, "mx_matmul: no LDS for the tile kernel");
+  static OncePerDevice once;
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return set_error(A8_ERR_HIP, "mx_matmul: no current device");
+  const int e = once(device, [] {
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(&k_mx_tile<FA, FB, MI, NI, KG, T>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, MxStage<FA, FB, MI, NI, KG>::kLds);
+  });
+  if (e != 0) return set_error(A8_ERR_HIP, "mx_matmul: no LDS for the tile kernel");
   const int64_t t = ((m + 64 * MI - 1) / (64 * MI)) * ((n + 64 * NI - 1) / (64 * NI));
   k_mx_tile<FA, FB, MI, NI, KG, T><<<(uint32_t)t, 256 * KG, lds, st>>>(a, sa, b, sb, c, m, n, k);
   return check_launch("k_mx_tile");
