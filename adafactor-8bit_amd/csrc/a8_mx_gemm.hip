@@ -146,14 +146,18 @@ __device__ __forceinline__ i32x4 mx_buffer(const uint8_t* p, int64_t bytes) {
   return r;
 }
 
-// 16 bytes a lane from buffer + off to LDS at lds + 16 * lane.  No register is written, and
-// the caller waits (vmcnt) before it reads the LDS.
+// 16 bytes a lane from buffer + off to LDS at lds + 16 * lane.  No register is written but m0, and
+// the caller waits (vmcnt) before it reads the LDS.  The compiler sets m0 before a use of its own and may join
+// such settings; m0 is named so that it joins none across the block (the warning: nothing saves m0 here).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void mx_to_lds(i32x4 buf, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds), "v"(off), "s"(buf)
-               : "memory");
+               : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 template <int N>
 __device__ __forceinline__ void mx_wait_barrier() {   // own loads to LDS but the last N, own LDS reads; then everyone's
