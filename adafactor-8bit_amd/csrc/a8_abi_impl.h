@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "../../include/adafactor8bit_amd.h"
+#include "a8_launch.h"
 
 namespace a8 {
 

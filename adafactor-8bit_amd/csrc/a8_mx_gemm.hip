@@ -495,6 +495,7 @@ int tiles(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* 
   });
   if (e != 0) return set_error(A8_ERR_HIP, "mx_matmul: no LDS for the tile kernel");
   const int64_t t = ((m + 64 * MI - 1) / (64 * MI)) * ((n + 64 * NI - 1) / (64 * NI));
+  if (t > most_groups(256 * KG)) return set_error(A8_ERR_SIZE, "mx_matmul: more tiles than one launch takes");
   k_mx_tile<FA, FB, MI, NI, KG, T><<<(uint32_t)t, 256 * KG, lds, st>>>(a, sa, b, sb, c, m, n, k);
   return check_launch("k_mx_tile");
 }
@@ -503,6 +504,7 @@ template <int FA, int FB, typename T>
 int few(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, T* c, int64_t m, int64_t n,
         int64_t k, hipStream_t st) {
   const int64_t g = (n + 31) / 32;
+  if (g > most_groups(256)) return set_error(A8_ERR_SIZE, "mx_matmul: more rows of b than one launch takes");
   // Fewer tiles than CUs take eight waves each.  Where every CU has several in turn memory's rate is the
   // bound, and a steady stream reads faster than bursts (1 x 128256 x 4096, 8 by 4 bits: 55 us against 65;
   // 1 x 14336 x 4096 the other way, 8.6 against 8.0).
@@ -517,8 +519,10 @@ int matmul(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t*
            int64_t k, hipStream_t st) {
   T* o = static_cast<T*>(c);
   if (k == 0) {
-    k_mx_zero<T><<<(uint32_t)((m * n + 255) / 256), 256, 0, st>>>(o, m * n);
-    return check_launch("k_mx_zero");
+    return in_runs(m * n, most_groups(256) * 256, [&](int64_t first, int64_t count) {
+      k_mx_zero<T><<<(uint32_t)((count + 255) / 256), 256, 0, st>>>(o + first, count);
+      return check_launch("k_mx_zero");
+    });
   }
   // Few rows: a workgroup reads all of a from the L2 beside its rows of b, so the more rows a has, the more
   // the tiles save that read it once for 64 of them, if there are tiles enough (24 x 32000 x 2048, 8 by 4 bits: 9.1

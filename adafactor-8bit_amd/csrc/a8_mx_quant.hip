@@ -210,8 +210,9 @@ int quantize(const T* x, int64_t rows, int64_t cols, int64_t stride, uint8_t* co
     const int64_t down = mx_pitch(rows) / 128;
     auto go = [&](auto along, auto cw) {
       constexpr int CW = decltype(cw)::value;
-      const uint32_t g = (uint32_t)(down * (mx_pitch(cols) / (128 * CW)));
-      k_mx_both<T, FMT, SR, decltype(along)::value, CW><<<g, 256 * CW, 0, st>>>(
+      const int64_t g = down * (mx_pitch(cols) / (128 * CW));
+      if (g > most_groups(256 * CW)) return set_error(A8_ERR_SIZE, "mx_quantize: more tiles than one launch takes");
+      k_mx_both<T, FMT, SR, decltype(along)::value, CW><<<(uint32_t)g, 256 * CW, 0, st>>>(
           x, stride, rows, cols, codes, scales, codes_t, scales_t, ceil, base, base_t, (uint32_t)down);
       return check_launch("k_mx_both");
     };
@@ -225,9 +226,14 @@ int quantize(const T* x, int64_t rows, int64_t cols, int64_t stride, uint8_t* co
     };
     return codes ? way(std::true_type{}) : way(std::false_type{});
   }
-  const int64_t lanes = rows * (mx_pitch(cols) / 8);
-  k_mx_rows<T, FMT, SR><<<(uint32_t)((lanes + 255) / 256), 256, 0, st>>>(x, stride, rows, cols, codes, scales, ceil, base);
-  return check_launch("k_mx_rows");
+  const int64_t pitch = mx_pitch(cols);
+  return in_runs(rows, most_groups(256) * 256 / (pitch / 8), [&](int64_t first, int64_t count) {
+    const int64_t e = first * pitch;
+    k_mx_rows<T, FMT, SR><<<(uint32_t)((count * (pitch / 8) + 255) / 256), 256, 0, st>>>(
+        x + first * stride, stride, count, cols, codes + (FMT == kFp8 ? e : e / 2), scales + e / 32, ceil,
+        base + (uint64_t)e / 4);
+    return check_launch("k_mx_rows");
+  });
 }
 
 template <typename T>
@@ -287,13 +293,20 @@ extern "C" int a8_mx_dequantize(int dtype, int fmt, void* out, const uint8_t* co
   if (!out || !codes || !scales) return set_error(A8_ERR_ARG, "mx_dequantize: null pointer");
   if (!aligned16(codes)) return set_error(A8_ERR_ALIGN, "mx_dequantize: codes must be 16-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const uint32_t g = (uint32_t)((rows * ((cols + 7) / 8) + 255) / 256);
-#define A8_READ(T)                                                                                              \
-  if (fmt == A8_MXFP4) k_mx_read<T, kFp4><<<g, 256, 0, st>>>(static_cast<T*>(out), codes, scales, rows, cols); \
-  else k_mx_read<T, kFp8><<<g, 256, 0, st>>>(static_cast<T*>(out), codes, scales, rows, cols)
-  if (dtype == A8_F32) { A8_READ(float); }
-  else if (dtype == A8_BF16) { A8_READ(__hip_bfloat16); }
-  else { A8_READ(__half); }
-#undef A8_READ
-  return check_launch("k_mx_read");
+  auto go = [&](auto* o) {
+    typedef std::remove_pointer_t<decltype(o)> T;
+    const int64_t pitch = mx_pitch(cols), per = (cols + 7) / 8;
+    return in_runs(rows, most_groups(256) * 256 / per, [&](int64_t first, int64_t count) {
+      const uint32_t g = (uint32_t)((count * per + 255) / 256);
+      const int64_t e = first * pitch;
+      if (fmt == A8_MXFP4)
+        k_mx_read<T, kFp4><<<g, 256, 0, st>>>(o + first * cols, codes + e / 2, scales + e / 32, count, cols);
+      else
+        k_mx_read<T, kFp8><<<g, 256, 0, st>>>(o + first * cols, codes + e, scales + e / 32, count, cols);
+      return check_launch("k_mx_read");
+    });
+  };
+  if (dtype == A8_F32) return go(static_cast<float*>(out));
+  if (dtype == A8_BF16) return go(static_cast<__hip_bfloat16*>(out));
+  return go(static_cast<__half*>(out));
 }

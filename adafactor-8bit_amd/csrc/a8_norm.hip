@@ -426,16 +426,29 @@ constexpr int64_t kLong = 32768, kLongBwd = 16384;
 template <typename T, typename R, typename W, int OUT>
 int rms_out(const T* x, int64_t xs, const R* r, int64_t rs, const W* w, T* y, uint8_t* codes, uint8_t* scales, R* h,
             uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps, hipStream_t st) {
-  const int64_t wide = OUT ? mx_pitch(cols) : cols;
-  if (wide > kLong) {
-    k_rms_long<T, R, W, OUT><<<(uint32_t)rows, 1024, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd, cols, eps);
-    return check_launch("k_rms_long");
-  }
+  const int64_t pitch = mx_pitch(cols), wide = OUT ? pitch : cols;
+  // `most` rows a launch: f(first row, rows, the arrays from the first row on)
+  auto go = [&](int64_t most, auto&& f) {
+    return in_runs(rows, most, [&](int64_t first, int64_t count) {
+      const int64_t e = first * pitch;
+      return f(count, x + first * xs, r ? r + first * rs : nullptr, y ? y + first * cols : nullptr,
+               codes ? codes + (OUT == 1 + kFp8 ? e : e / 2) : nullptr, scales ? scales + e / 32 : nullptr,
+               h ? h + first * cols : nullptr, low ? low + first * ((cols + 7) / 8) : nullptr,
+               rstd ? rstd + first : nullptr);
+    });
+  };
+  if (wide > kLong)
+    return go(most_groups(1024), [&](int64_t n, auto x, auto r, auto y, auto codes, auto scales, auto h, auto low, auto rstd) {
+      k_rms_long<T, R, W, OUT><<<(uint32_t)n, 1024, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd, cols, eps);
+      return check_launch("k_rms_long");
+    });
   return with_shape<true>(wide, [&](auto tpr, auto nc) {
     constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, B = TPR < 256 ? 256 : TPR, K = B / TPR;
-    k_rms<T, R, W, OUT, TPR, NC><<<(uint32_t)((rows + K - 1) / K), B, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd,
-                                                                               rows, cols, eps);
-    return check_launch("k_rms");
+    return go(most_groups(B) * K, [&](int64_t n, auto x, auto r, auto y, auto codes, auto scales, auto h, auto low, auto rstd) {
+      k_rms<T, R, W, OUT, TPR, NC><<<(uint32_t)((n + K - 1) / K), B, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd,
+                                                                              n, cols, eps);
+      return check_launch("k_rms");
+    });
   });
 }
 
@@ -533,7 +546,7 @@ extern "C" int a8_rms_norm_backward(int dtype, int res_dtype, int w_dtype, const
                                     float* workspace, int64_t rows, int64_t cols, void* stream) {
   if (int e = check_types(dtype, res_dtype, w_dtype, "rms_norm_backward: dy must be fp32, bf16 or fp16, the residual and "
                                                      "the weight of that type or fp32")) return e;
-  if (rows < 0 || rows >= kLim || cols < 1 || cols >= kLim)
+  if (rows < 0 || rows >= kLim || cols < 1 || (cols + 31) / 32 > most_groups(1024))   // k_rms_dw's workgroups
     return set_error(A8_ERR_SIZE, "rms_norm_backward: rows or cols out of range");
   if (!dw || (rows > 0 && (!dy || !h || !weight || !rstd || !dx || !workspace)))
     return set_error(A8_ERR_ARG, "rms_norm_backward: null pointer");

@@ -815,7 +815,8 @@ int64_t a8_mx_pitch(int64_t cols);
  * stochastic != 0, up with the probability of their distance: floor(t / step + (u + 1/2) /
  * 2^16) in fp32, t the scaled magnitude, step the grid's at t, u 16 bits of
  * SplitMix64(seed * 0x9E3779B97F4A7C15 + (0 | 0xD1B54A32D192ED03 for the transpose)
- * + i / 4) for element i of the padded output, the (i % 4)-th from the low end. */
+ * + i / 4) for element i of the padded output, the (i % 4)-th from the low end.
+ * Sizes below 2^31; with codes_t fewer than 2^24 - 1 tiles of 128 x 128. */
 int a8_mx_quantize(int dtype, int fmt, int scale_rule, int stochastic, const void* x, int64_t rows, int64_t cols,
                    int64_t row_stride, uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t,
                    uint64_t seed, void* stream);
@@ -826,7 +827,8 @@ int a8_mx_dequantize(int dtype, int fmt, void* out, const uint8_t* codes, const 
 
 /* c [m, n] (contiguous, out_dtype fp32, bf16 or fp16) = a b^T for MX tensors a [m, k]
  * and b [n, k] of either format, accumulated in fp32 and rounded once.  Sizes below 2^31, k
- * below 2^23; operands and c start on 16-byte boundaries. */
+ * below 2^23, fewer than 2^24 tiles of 128 x 128 (up to 32 rows of a: n at most 2^29 - 32);
+ * operands and c start on 16-byte boundaries. */
 int a8_mx_matmul(int fmt_a, int fmt_b, int out_dtype, const uint8_t* a_codes, const uint8_t* a_scales,
                  const uint8_t* b_codes, const uint8_t* b_scales, void* c, int64_t m, int64_t n, int64_t k,
                  void* stream);
@@ -846,7 +848,7 @@ int a8_rms_norm(int dtype, int res_dtype, int w_dtype, int out_fmt, const void* 
  * or NULL) and the h, h_low (NULL: h as it is) and rstd of the forward pass: dx = s (dy w - h s mean(dy w h s)) +
  * dh, the same in dr (of h's type; NULL: not written), and dw = sum over rows of dy h s,
  * in the weight's type, summed in a fixed order.  workspace:
- * a8_rms_norm_workspace_floats(rows, cols) floats. */
+ * a8_rms_norm_workspace_floats(rows, cols) floats.  cols at most 2^27 - 32. */
 int a8_rms_norm_backward(int dtype, int res_dtype, int w_dtype, const void* dy, const void* dh, const void* h,
                          const uint32_t* h_low, const void* weight, const float* rstd, void* dx, void* dr, void* dw, float* workspace,
                          int64_t rows, int64_t cols, void* stream);
