@@ -14,6 +14,7 @@ would saturate (``scale="ceil"``).  A block that holds a NaN or an infinity read
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -123,6 +124,14 @@ def _on_gpu(x, what):
         raise RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got a tensor on {x.device}")
 
 
+def no_tangents(what, *tensors):
+    """A launch that autograd does not see carries no tangent on: its result would read as a constant."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"adafactor8bit: {what} has no forward-mode derivative, got a dual tensor")
+
+
 def _not_on_gpu(t, what):
     return RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got an MX tensor on {t.keep[0].device} and {t.keep[-1].device}")
 
@@ -182,6 +191,7 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
     if x.dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_quantize takes fp32, bf16 or fp16, got {x.dtype}")
     _on_gpu(x, "mx_quantize")
+    no_tangents("mx_quantize", x)
     if axis not in (0, 1, "both"):
         raise ValueError(f"adafactor8bit: axis must be 0, 1 or 'both', got {axis!r}")
     a, d = _quantize(_rows(x.detach()), fmt, f, axis != 0, axis != 1, rule, seed)
@@ -232,6 +242,7 @@ def first_order(name, gradients):
     def backward(ctx, *dy):
         if torch.is_grad_enabled():
             raise RuntimeError(f"adafactor8bit: {name} cannot be differentiated twice; call without create_graph")
+        no_tangents(f"{name}'s backward pass", *dy)
         return plain(ctx, *dy)
 
     return staticmethod(backward)
@@ -271,7 +282,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     the rows.  For the backward pass only the transposed blocks are kept.  ``seed``: a whole number
     rounds dy stochastically (pass another one each step); None rounds to nearest.  ``scale`` is the
     rule of every operand; "ceil" saturates nothing, so that stochastic rounding has no bias.  The gradients
-    have none themselves: ``create_graph`` is refused.
+    have none themselves: ``create_graph`` is refused, and so are forward-mode derivatives.
 
     ``weight`` may be an MXTensor laid out once (serving): x is then quantised and multiplied, without
     gradients.
@@ -285,6 +296,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     if x.dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16, got {x.dtype}")
     _on_gpu(x, "mx_linear")
+    no_tangents("mx_linear", x, None if isinstance(weight, MXTensor) else weight)
     if isinstance(weight, MXTensor):
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError("adafactor8bit: mx_linear with a weight in MX blocks has no backward pass")

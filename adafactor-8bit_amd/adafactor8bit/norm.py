@@ -6,7 +6,7 @@ optimizer holds, writing the 8-bit activations that ``mx_matmul`` reads.
 import torch
 
 from . import _native as nat
-from .mx import _DTYPE, _FMT, _code, _launch, _new, _on_gpu, _rows, first_order
+from .mx import _DTYPE, _FMT, _code, _launch, _new, _on_gpu, _rows, first_order, no_tangents
 
 _DENSE = torch.contiguous_format
 
@@ -66,7 +66,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None):
     x is fp32, bf16 or fp16; ``weight`` [cols] and ``residual`` (x's shape) have x's type or fp32; y has
     x's type, h the residual's.  The sum enters the norm, and its gradients, before it is
     rounded to h's type (the gradients: to four bits more than a 16-bit h has, half a byte an element kept for them);
-    the gradients have none themselves: ``create_graph`` is refused.  ``out_fmt``
+    the gradients have none themselves: ``create_graph`` is refused, as forward-mode derivatives are.  ``out_fmt``
     "mxfp8" or "mxfp4": y is an MXTensor [rows, cols] (leading dimensions flattened) for ``mx_matmul``,
     without gradients.
     """
@@ -87,6 +87,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None):
             raise ValueError(f"adafactor8bit: rms_norm of x {tuple(shape)} with residual {tuple(residual.shape)}")
         if residual.dtype != dtype and residual.dtype != torch.float32:
             raise TypeError(f"adafactor8bit: rms_norm's residual is {dtype} or fp32, got {residual.dtype}")
+    no_tangents("rms_norm", x, weight, residual)
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                         or (residual is not None and residual.requires_grad))
     if grad and out_fmt is not None:

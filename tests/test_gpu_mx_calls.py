@@ -1,0 +1,38 @@
+"""Calls of the microscaled operators and the norm under autograd's and the tracers' modes: what has no
+derivative or no graph is refused, and what a mode does not ask for is not computed."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import adafactor8bit as a8
+
+pytestmark = pytest.mark.gpu
+
+
+def _r(m, k, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(m, k, generator=g) * scale).to(dtype).cuda()
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be dropped: the result would read as one that does not depend on its input."""
+    x, w, g = _r(8, 64, 1), _r(16, 64, 2), _r(1, 64, 3)[0]
+    q = a8.mx_quantize(w, "mxfp4")
+    with fwd.dual_level():
+        d, dw, dg = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w, g))
+        for f in (lambda: a8.rms_norm(d, g), lambda: a8.rms_norm(x, dg), lambda: a8.rms_norm(x, g, residual=d),
+                  lambda: a8.rms_norm(d, g, out_fmt="mxfp8"), lambda: a8.mx_quantize(d), lambda: a8.mx_linear(d, q),
+                  lambda: a8.mx_linear(d, w), lambda: a8.mx_linear(x, dw),
+                  lambda: a8.mx_linear(d.clone().requires_grad_(), w)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+        assert torch.isfinite(a8.rms_norm(x, g)).all()          # without a tangent the level changes nothing
+        r = x.clone().requires_grad_()
+        for f in (lambda: a8.rms_norm(r, g), lambda: a8.mx_linear(r, w), lambda: a8.rms_norm(r, g, residual=r)[1]):
+            y = f()
+            assert torch.isfinite(torch.autograd.grad(y, r, torch.ones_like(y), retain_graph=True)[0]).all()
+            with pytest.raises(RuntimeError, match="forward-mode"):   # nor does a gradient have a tangent
+                torch.autograd.grad(y, r, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    assert a8.mx_linear(x, q).shape == (8, 16)
