@@ -3,6 +3,7 @@ derivative or no graph is refused, and what a mode does not ask for is not compu
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import adafactor8bit as a8
 
@@ -36,3 +37,17 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):   # nor does a gradient have a tangent
                 torch.autograd.grad(y, r, fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
     assert a8.mx_linear(x, q).shape == (8, 16)
+
+
+def test_tracing_is_refused():
+    """A trace would hold the outputs' allocation and not the launch that writes them."""
+    x, w, g = _r(8, 64, 1), _r(16, 64, 2), _r(1, 64, 3)[0]
+    q = a8.mx_quantize(w, "mxfp4")
+    for f in (lambda t: a8.rms_norm(t, g), lambda t: a8.rms_norm(t, g, residual=t)[0], lambda t: a8.mx_linear(t, w),
+              lambda t: a8.mx_linear(t, q), lambda t: a8.mx_dequantize(a8.mx_quantize(t))):
+        want = f(x)
+        for trace in (lambda: torch.jit.trace(f, (x,), check_trace=False), lambda: make_fx(f)(x),
+                      lambda: make_fx(f, pre_dispatch=True)(x)):
+            with pytest.raises(RuntimeError, match="trace"):
+                trace()
+        assert torch.equal(f(x), want)
