@@ -32,8 +32,8 @@ def _code(table, key, what):
         raise ValueError(f"adafactor8bit: {what} must be one of {', '.join(map(str, table))}, got {key!r}") from None
 
 
-def _pitch(cols):
-    return (cols + 255) & -256
+def _pitch(cols):   # no shifts or masks here and in _bytes: torch.compile's symbolic sizes have none
+    return (cols + 255) // 256 * 256
 
 
 class MXTensor:
@@ -71,7 +71,7 @@ class MXTensor:
         codes = keep[0]
         at = codes.data_ptr()
         if len(keep) == 1:
-            return at, at + self.rows * ((self.cols + 255 & -256) >> (1 - self.f)), codes.get_device()
+            return at, at + self.rows * (_pitch(self.cols) // (2 - self.f)), codes.get_device()
         i = codes.get_device()
         return at, keep[1].data_ptr(), i if keep[1].get_device() == i else -1
 
@@ -112,7 +112,7 @@ def _over(buf, rows, cols, fmt, f):
 
 def _bytes(rows, cols, f):
     p = _pitch(cols)
-    return rows * ((p >> (1 - f)) + (p >> 5))
+    return rows * (p // (2 - f) + p // 32)
 
 
 def _new(rows, cols, fmt, f, device):

@@ -51,3 +51,27 @@ def test_tracing_is_refused():
             with pytest.raises(RuntimeError, match="trace"):
                 trace()
         assert torch.equal(f(x), want)
+
+
+@pytest.mark.parametrize("rows", [(8,), (8, 12, 5)])
+def test_compiled_programs_call_the_operators(rows):
+    """torch.compile runs the operators between its graphs, also where it makes sizes symbolic."""
+    w, g = _r(16, 64, 2), _r(1, 64, 3)[0]
+    q = a8.mx_quantize(w, "mxfp4")
+    for f in (lambda t: a8.rms_norm(t * 2, g) + 1, lambda t: a8.mx_linear(t * 2, w) + 1, lambda t: a8.mx_linear(t * 2, q) + 1,
+              lambda t: a8.mx_linear(t * 2, w, "mxfp4", "mxfp8", "mxfp4", seed=3) + 1,
+              lambda t: a8.mx_dequantize(a8.mx_quantize(t * 2)) + 1):
+        torch._dynamo.reset()
+        c = torch.compile(f, backend="eager")
+        for m in rows:
+            x = _r(m, 64, m)
+            with torch.no_grad():
+                assert torch.equal(c(x), f(x))
+    for f in (lambda t: a8.rms_norm(t * 2, g) + 1, lambda t: a8.mx_linear(t * 2, w) + 1):
+        torch._dynamo.reset()
+        c = torch.compile(f, backend="eager")
+        for m in rows:
+            x = _r(m, 64, m).requires_grad_()
+            y, z = c(x), f(x)
+            assert torch.equal(y, z)
+            assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.autograd.grad(z, x, torch.ones_like(z))[0])
