@@ -190,7 +190,8 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
     x's columns (what a product over x's rows reads).  ``axis="both"``: the pair, from one reading.
     ``seed``: None rounds to the nearest code, ties to even; a whole number rounds up with the
     probability of the distance, by the optimizer's counter stream for that seed (other seeds, other
-    draws; the same seed, the same codes).
+    draws; the same seed, the same codes).  An MX tensor has no gradient: an x that requires one is refused
+    where gradients are recorded.
     """
     f, rule = _code(_FMT, fmt, "fmt"), _code(_RULE, scale, "scale")
     if x.dim() < 1:
@@ -201,7 +202,9 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
     no_tangents("mx_quantize", x)
     if axis not in (0, 1, "both"):
         raise ValueError(f"adafactor8bit: axis must be 0, 1 or 'both', got {axis!r}")
-    a, d = _quantize(_rows(x.detach()), fmt, f, axis != 0, axis != 1, rule, seed)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("adafactor8bit: an MX tensor has no gradient; call mx_quantize under torch.no_grad() or on x.detach()")
+    a, d = _quantize(_rows(x), fmt, f, axis != 0, axis != 1, rule, seed)
     return (a, d) if axis == "both" else a if axis == 1 else d
 
 
@@ -309,7 +312,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
             raise ValueError("adafactor8bit: mx_linear with a weight in MX blocks has no backward pass")
         if weight.device != x.device:
             raise ValueError("adafactor8bit: mx_linear's operands are on one device")
-        xa, _ = _quantize(_rows(x.detach()), *fmts[0], True, False, rule, None)
+        xa, _ = _quantize(_rows(x), *fmts[0], True, False, rule, None)
         y = _matmul(xa, weight, x.dtype, "mx_linear")
     else:
         if weight.dtype not in _DTYPE:

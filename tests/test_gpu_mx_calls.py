@@ -53,6 +53,17 @@ def test_tracing_is_refused():
         assert torch.equal(f(x), want)
 
 
+def test_quantize_keeps_no_gradient_and_says_so():
+    x = _r(8, 64, 1).requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        a8.mx_quantize(x)
+    want = a8.mx_quantize(x.detach(), axis="both")
+    with torch.no_grad():
+        got = a8.mx_quantize(x, axis="both")
+    for a, b in zip(got, want):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
 @pytest.mark.parametrize("rows", [(8,), (8, 12, 5)])
 def test_compiled_programs_call_the_operators(rows):
     """torch.compile runs the operators between its graphs, also where it makes sizes symbolic."""
