@@ -307,17 +307,17 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
         raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16, got {x.dtype}")
     _on_gpu(x, "mx_linear")
     no_tangents("mx_linear", x, None if isinstance(weight, MXTensor) else weight)
-    if isinstance(weight, MXTensor):
-        if x.requires_grad and torch.is_grad_enabled():
+    if weight.device != x.device:
+        raise ValueError("adafactor8bit: mx_linear's operands are on one device")
+    blocks = isinstance(weight, MXTensor)
+    if not blocks and weight.dtype not in _DTYPE:
+        raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16 weights, got {weight.dtype}")
+    if torch.is_grad_enabled() and (x.requires_grad or (not blocks and weight.requires_grad)):
+        if blocks:
             raise ValueError("adafactor8bit: mx_linear with a weight in MX blocks has no backward pass")
-        if weight.device != x.device:
-            raise ValueError("adafactor8bit: mx_linear's operands are on one device")
-        xa, _ = _quantize(_rows(x), *fmts[0], True, False, rule, None)
-        y = _matmul(xa, weight, x.dtype, "mx_linear")
-    else:
-        if weight.dtype not in _DTYPE:
-            raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16 weights, got {weight.dtype}")
-        if weight.device != x.device:
-            raise ValueError("adafactor8bit: mx_linear's operands are on one device")
         y = _Linear.apply(_rows(x), _rows(weight), fmts, rule, seed)
+    else:   # no gradients: along the rows alone
+        xa, _ = _quantize(_rows(x), *fmts[0], True, False, rule, None)
+        wa = weight if blocks else _quantize(_rows(weight), *fmts[1], True, False, rule, None)[0]
+        y = _matmul(xa, wa, x.dtype, "mx_linear")
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.shape[0])

@@ -6,6 +6,8 @@ import torch.autograd.forward_ad as fwd
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import adafactor8bit as a8
+from adafactor8bit import mx as mxmod
+from adafactor8bit import norm as normmod
 
 pytestmark = pytest.mark.gpu
 
@@ -13,6 +15,19 @@ pytestmark = pytest.mark.gpu
 def _r(m, k, seed, dtype=torch.float32, scale=1.0):
     g = torch.Generator().manual_seed(seed)
     return (torch.randn(m, k, generator=g) * scale).to(dtype).cuda()
+
+
+def _calls(monkeypatch):
+    """The library's calls from here on, as (name, arguments)."""
+    seen, real = [], mxmod._launch
+
+    def launch(name, device, *args):
+        seen.append((name, args))
+        return real(name, device, *args)
+
+    monkeypatch.setattr(mxmod, "_launch", launch)
+    monkeypatch.setattr(normmod, "_launch", launch)
+    return seen
 
 
 def test_forward_mode_is_refused():
@@ -62,6 +77,19 @@ def test_quantize_keeps_no_gradient_and_says_so():
         got = a8.mx_quantize(x, axis="both")
     for a, b in zip(got, want):
         assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_linear_without_gradients_quantises_along_the_rows_alone(mode, monkeypatch):
+    x, w = _r(24, 96, 1, torch.bfloat16).requires_grad_(), _r(40, 96, 2, torch.bfloat16).requires_grad_()
+    want = a8.mx_linear(x, w)
+    assert want.requires_grad
+    seen = _calls(monkeypatch)
+    with mode():
+        y = a8.mx_linear(x, w)
+    assert torch.equal(y, want) and not y.requires_grad
+    assert [n for n, _ in seen] == ["a8_mx_quantize", "a8_mx_quantize", "a8_mx_matmul"]
+    assert all(a[10] is None and a[11] is None for _, a in seen[:2])   # codes and scales of the transpose
 
 
 @pytest.mark.parametrize("rows", [(8,), (8, 12, 5)])
