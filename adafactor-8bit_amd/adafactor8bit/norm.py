@@ -40,9 +40,11 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def gradients(ctx, dy, dh=None):
+        if dy is None:   # h alone was used: its gradient, as it is
+            return (None, None, None, None) if dh is None else (dh.to(ctx.dtype), dh, None, None)
         h, low, weight, rstd = ctx.saved_tensors
         rows, cols = h.shape
-        dy = torch.zeros((rows, cols), dtype=ctx.dtype, device=h.device) if dy is None else dy.contiguous()
+        dy = dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty_like(dy)
         dr = torch.empty_like(h) if ctx.residual and h.dtype != ctx.dtype else None

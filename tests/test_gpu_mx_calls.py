@@ -92,6 +92,20 @@ def test_linear_without_gradients_quantises_along_the_rows_alone(mode, monkeypat
     assert all(a[10] is None and a[11] is None for _, a in seen[:2])   # codes and scales of the transpose
 
 
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+def test_the_residual_alone_passes_its_gradient_through(types):
+    """Where only h is used its gradient is dh itself, also in a row with infinities or NaN."""
+    tx, tr = types
+    x, r = _r(5, 40, 1, tx), _r(5, 40, 2, tr)
+    x[0, 3], x[1, 4], r[2, 5] = float("inf"), float("nan"), -float("inf")
+    x, r, w = x.requires_grad_(), r.requires_grad_(), torch.ones(40, device="cuda", dtype=tx, requires_grad=True)
+    dh = _r(5, 40, 3, tr)
+    _, h = a8.rms_norm(x, w, residual=r)
+    gx, gr, gw = torch.autograd.grad(h, (x, r, w), dh, allow_unused=True)
+    assert gx.dtype == tx and torch.equal(gx, dh.to(tx)) and torch.equal(gr, dh)
+    assert gw is None or not gw.any()
+
+
 @pytest.mark.parametrize("rows", [(8,), (8, 12, 5)])
 def test_compiled_programs_call_the_operators(rows):
     """torch.compile runs the operators between its graphs, also where it makes sizes symbolic."""
