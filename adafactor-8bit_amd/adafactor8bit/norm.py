@@ -48,12 +48,15 @@ class _RmsNorm(torch.autograd.Function):
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty_like(dy)
         dr = torch.empty_like(h) if ctx.residual and h.dtype != ctx.dtype else None
-        dw = torch.empty_like(weight)
-        ws = rstd.new_empty(nat.lib().a8_rms_norm_workspace_floats(rows, cols))
+        dw = ws = None
+        if ctx.needs_input_grad[2]:   # a frozen weight's gradient is not summed
+            dw = torch.empty_like(weight)
+            ws = rstd.new_empty(nat.lib().a8_rms_norm_workspace_floats(rows, cols))
         _launch("a8_rms_norm_backward", h.get_device(), _DTYPE[ctx.dtype], _DTYPE[h.dtype], _DTYPE[weight.dtype], dy.data_ptr(),
                 None if dh is None else dh.data_ptr(), h.data_ptr(),
                 None if low is None else low.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-                None if dr is None else dr.data_ptr(), dw.data_ptr(), ws.data_ptr(), rows, cols)
+                None if dr is None else dr.data_ptr(), None if dw is None else dw.data_ptr(),
+                None if ws is None else ws.data_ptr(), rows, cols)
         if not ctx.residual:
             return dx, None, dw, None
         return dx, dx if dr is None else dr, dw, None

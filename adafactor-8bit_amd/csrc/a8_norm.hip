@@ -223,7 +223,7 @@ __global__ __launch_bounds__(1024) void k_rms_long(const T* x, int64_t xs, const
 // keeps its columns of the weight and of dw's sum in registers, and asks for its next row before this one's sum
 // is known: without that 16384 x 4096 bf16 with a residual takes 165 us, with it 117 (4.6 TB/s), bound by memory;
 // 124 with the bits below h.
-// parts [grid, cols]: each workgroup's dw.
+// parts [grid, cols]: each workgroup's dw (NULL: none).
 template <typename T, typename R, typename W, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_bwd(const T* dy, const R* dh, const R* h, const uint32_t* low,
                                                  const W* w, const float* rstd, T* dx, R* dr, float* parts,
@@ -300,6 +300,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_bwd(const T* dy, 
       }
     }
   }
+  if (!parts) return;      // the weight's gradient is not wanted
   if constexpr (K > 1) {   // the waves' sums, in their order
     __shared__ __align__(16) float all[K][8 * TPR];
 #pragma unroll
@@ -330,7 +331,8 @@ __global__ __launch_bounds__(1024) void k_rms_bwd_long(const T* dy, const R* dh,
                                                        int64_t cols) {
   __shared__ float lds[2][16];
   int turn = 0;
-  parts += (int64_t)blockIdx.x * cols;
+  const bool sums = parts != nullptr;
+  if (sums) parts += (int64_t)blockIdx.x * cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const float s = rstd[row];
     float sum = 0.0f;
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(1024) void k_rms_bwd_long(const T* dy, const R* dh,
       load8(h + row * cols, c, cols, v);
       if constexpr (kLow<R>) add_low<R>(get_low(low, row, c, cols), v);
       load8(w, c, cols, u);
-      if (row != blockIdx.x) load8(parts, c, cols, d);
+      if (sums && row != blockIdx.x) load8(parts, c, cols, d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float xn = v[i] * s;
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(1024) void k_rms_bwd_long(const T* dy, const R* dh,
         d[i] = row == blockIdx.x ? g[i] * xn : d[i] + g[i] * xn;
       }
       sum += part;
-      store8(parts, c, cols, d);
+      if (sums) store8(parts, c, cols, d);
     }
     sum = row_sum<1024>(sum, lds[turn]) / (float)cols;
     for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += 8192) {
@@ -469,6 +471,7 @@ template <typename T, typename R, typename W>
 int rms_bwd(const void* dy_, const void* dh_, const void* h_, const uint32_t* low, const void* w_, const float* rstd,
             void* dx_, void* dr_, void* dw, float* parts, int64_t rows, int64_t cols, hipStream_t st) {
   const int n = bwd_groups(rows, cols);
+  if (!dw) parts = nullptr;
   const T* dy = static_cast<const T*>(dy_);
   const R *dh = static_cast<const R*>(dh_), *h = static_cast<const R*>(h_);
   const W* w = static_cast<const W*>(w_);
@@ -485,7 +488,7 @@ int rms_bwd(const void* dy_, const void* dh_, const void* h_, const uint32_t* lo
       return check_launch("k_rms_bwd");
     });
   }
-  if (e) return e;
+  if (e || !dw) return e;
   k_rms_dw<W><<<(uint32_t)((cols + 31) / 32), 1024, 0, st>>>(parts, static_cast<W*>(dw), cols, n);
   return check_launch("k_rms_dw");
 }
@@ -548,7 +551,7 @@ extern "C" int a8_rms_norm_backward(int dtype, int res_dtype, int w_dtype, const
                                                      "the weight of that type or fp32")) return e;
   if (rows < 0 || rows >= kLim || cols < 1 || (cols + 31) / 32 > most_groups(1024))   // k_rms_dw's workgroups
     return set_error(A8_ERR_SIZE, "rms_norm_backward: rows or cols out of range");
-  if (!dw || (rows > 0 && (!dy || !h || !weight || !rstd || !dx || !workspace)))
+  if (rows > 0 && (!dy || !h || !weight || !rstd || !dx || (dw && !workspace)))
     return set_error(A8_ERR_ARG, "rms_norm_backward: null pointer");
   return with_types(dtype, res_dtype, w_dtype, [&](auto t, auto r, auto w) {
     return rms_bwd<decltype(t), decltype(r), decltype(w)>(dy, dh, h, h_low, weight, rstd, dx, dr, dw, workspace, rows, cols,

@@ -847,7 +847,7 @@ int a8_rms_norm(int dtype, int res_dtype, int w_dtype, int out_fmt, const void* 
 /* Gradients of a8_rms_norm for contiguous dy (x's type), dh (h's gradient, of h's type,
  * or NULL) and the h, h_low (NULL: h as it is) and rstd of the forward pass: dx = s (dy w - h s mean(dy w h s)) +
  * dh, the same in dr (of h's type; NULL: not written), and dw = sum over rows of dy h s,
- * in the weight's type, summed in a fixed order.  workspace:
+ * in the weight's type, summed in a fixed order (NULL: not wanted, and no workspace either).  workspace:
  * a8_rms_norm_workspace_floats(rows, cols) floats.  cols at most 2^27 - 32. */
 int a8_rms_norm_backward(int dtype, int res_dtype, int w_dtype, const void* dy, const void* dh, const void* h,
                          const uint32_t* h_low, const void* weight, const float* rstd, void* dx, void* dr, void* dw, float* workspace,

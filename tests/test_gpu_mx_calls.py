@@ -92,6 +92,21 @@ def test_linear_without_gradients_quantises_along_the_rows_alone(mode, monkeypat
     assert all(a[10] is None and a[11] is None for _, a in seen[:2])   # codes and scales of the transpose
 
 
+@pytest.mark.parametrize("dtype,k", [(torch.bfloat16, 300), (torch.float32, 3000), (torch.float16, 17000)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_with_a_frozen_gain_sums_no_gradient_of_it(dtype, k, residual, monkeypatch):
+    x, r, w = _r(9, k, 1, dtype).requires_grad_(), _r(9, k, 2, dtype), _r(1, k, 3, dtype)[0]
+    dy = _r(9, k, 4, dtype)
+    first = lambda o: o[0] if residual else o  # noqa: E731
+    f = lambda w: first(a8.rms_norm(x, w, residual=r if residual else None))  # noqa: E731
+    want = torch.autograd.grad(f(w.clone().requires_grad_()), x, dy)[0]
+    seen = _calls(monkeypatch)
+    got = torch.autograd.grad(f(w), x, dy)[0]
+    assert torch.equal(got, want)
+    name, args = seen[-1]
+    assert name == "a8_rms_norm_backward" and args[11] is None and args[12] is None   # dw and its workspace
+
+
 @pytest.mark.parametrize("types", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
 def test_the_residual_alone_passes_its_gradient_through(types):
     """Where only h is used its gradient is dh itself, also in a row with infinities or NaN."""
