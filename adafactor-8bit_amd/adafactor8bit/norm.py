@@ -6,12 +6,12 @@ optimizer holds, writing the 8-bit activations that ``mx_matmul`` reads.
 import torch
 
 from . import _native as nat
-from .mx import _DTYPE, _FMT, _code, _launch, _new, _on_gpu, _rows, first_order, no_tangents
+from .mx import _DTYPE, _FMT, _RULE, _code, _launch, _new, _on_gpu, _rows, first_order, no_tangents
 
 _DENSE = torch.contiguous_format
 
 
-def _forward(x, residual, weight, eps, fmt, keep):
+def _forward(x, residual, weight, eps, fmt, keep, rule=0):
     """(y or an MX tensor, h or None, and for a backward pass the bits below h or None, 1 / rms of each row)."""
     rows, cols = x.shape
     dev = x.device
@@ -21,7 +21,8 @@ def _forward(x, residual, weight, eps, fmt, keep):
     low = h.new_empty((rows, (cols + 7) // 8), dtype=torch.int32) if keep and h is not None and h.element_size() == 2 else None
     rstd = x.new_empty(rows, dtype=torch.float32) if keep else None
     t = _DTYPE[x.dtype]
-    _launch("a8_rms_norm", x.get_device(), t, t if h is None else _DTYPE[h.dtype], _DTYPE[weight.dtype], f, x.data_ptr(), x.stride(0),
+    _launch("a8_rms_norm", x.get_device(), t, t if h is None else _DTYPE[h.dtype], _DTYPE[weight.dtype],
+            f | nat.MX_CEIL if rule else f, x.data_ptr(), x.stride(0),
             None if h is None else residual.data_ptr(), 0 if h is None else residual.stride(0), weight.data_ptr(),
             *((y.data_ptr(), None, None) if fmt is None else (None, *y._addresses()[:2])),
             None if h is None else h.data_ptr(), None if low is None else low.data_ptr(),
@@ -64,7 +65,7 @@ class _RmsNorm(torch.autograd.Function):
     backward = first_order("rms_norm", gradients)
 
 
-def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None):
+def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None, scale="floor"):
     """``h = x + residual`` (h = x without one) and ``y = h / sqrt(mean(h^2) + eps) * weight`` over the
     last dimension.  Returns y, or (y, h) with a residual.
 
@@ -73,8 +74,9 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None):
     rounded to h's type (the gradients: to four bits more than a 16-bit h has, half a byte an element kept for them);
     the gradients have none themselves: ``create_graph`` is refused, as forward-mode derivatives are.  ``out_fmt``
     "mxfp8" or "mxfp4": y is an MXTensor [rows, cols] (leading dimensions flattened) for ``mx_matmul``,
-    without gradients.
+    without gradients, its blocks' scales by the rule ``scale`` ("floor" or "ceil", as mx_quantize has them).
     """
+    rule = _code(_RULE, scale, "scale")
     if out_fmt is not None:
         _code(_FMT, out_fmt, "out_fmt")
     shape, dtype, dev = x.shape, x.dtype, x.device
@@ -104,7 +106,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None):
         out = _RmsNorm.apply(x2, r2, w, eps)
         y, h = out if r2 is not None else (out, None)
     else:
-        y, h, _, _ = _forward(x2, r2, w, eps, out_fmt, False)
+        y, h, _, _ = _forward(x2, r2, w, eps, out_fmt, False, 0 if out_fmt is None else rule)
     if len(shape) != 2:
         y = y if out_fmt is not None else y.reshape(shape)
         h = None if h is None else h.reshape(shape)

@@ -123,13 +123,13 @@ __device__ __forceinline__ void add_low(uint32_t w, float* v) {
 // y = v w s of eight columns; OUT: 0 the input's type, 1 + format an MX tensor
 template <int OUT, typename T>
 __device__ __forceinline__ void put8(T* y, uint8_t* codes, uint8_t* scales, int64_t row, int64_t col, int64_t cols,
-                                     int64_t pitch, const float* v) {
+                                     int64_t pitch, const float* v, int ceil) {
   if constexpr (OUT == 0) {
     store8(y + row * cols, col, cols, v);
   } else {
     constexpr int FMT = OUT - 1;
     const int64_t e = row * pitch + col;
-    mx_put8<FMT, false>(v, false, 0, 0, codes + (FMT == kFp8 ? e : e / 2), scales + e / 32);
+    mx_put8<FMT, false>(v, ceil != 0, 0, 0, codes + (FMT == kFp8 ? e : e / 2), scales + e / 32);
   }
 }
 
@@ -139,7 +139,8 @@ __device__ __forceinline__ void put8(T* y, uint8_t* codes, uint8_t* scales, int6
 template <typename T, typename R, typename W, int OUT, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms(const T* x, int64_t xs, const R* r, int64_t rs, const W* w,
                                                                T* y, uint8_t* codes, uint8_t* scales, R* h,
-                                                               uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps) {
+                                                               uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps,
+                                                               int ceil) {
   __shared__ float lds[TPR / 64];
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
   const int t = threadIdx.x % TPR;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms(const T* x, int64
     const int64_t c = (i * TPR + t) * 8;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] * s) * u[i][j];
-    if (c < end) put8<OUT>(y, codes, scales, row, c, cols, pitch, v[i]);
+    if (c < end) put8<OUT>(y, codes, scales, row, c, cols, pitch, v[i], ceil);
   }
 }
 
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms(const T* x, int64
 template <typename T, typename R, typename W, int OUT>
 __global__ __launch_bounds__(1024) void k_rms_long(const T* x, int64_t xs, const R* r, int64_t rs, const W* w, T* y,
                                                    uint8_t* codes, uint8_t* scales, R* h, uint32_t* low, float* rstd,
-                                                   int64_t cols, float eps) {
+                                                   int64_t cols, float eps, int ceil) {
   __shared__ float lds[16];
   const int64_t row = blockIdx.x, pitch = mx_pitch(cols), end = OUT ? pitch : cols;
   x += row * xs;
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(1024) void k_rms_long(const T* x, int64_t xs, const
     load8(w, c, cols, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (v[i] * s) * u[i];
-    put8<OUT>(y, codes, scales, row, c, cols, pitch, v);
+    put8<OUT>(y, codes, scales, row, c, cols, pitch, v, ceil);
   }
 }
 
@@ -427,7 +428,7 @@ constexpr int64_t kLong = 32768, kLongBwd = 16384;
 
 template <typename T, typename R, typename W, int OUT>
 int rms_out(const T* x, int64_t xs, const R* r, int64_t rs, const W* w, T* y, uint8_t* codes, uint8_t* scales, R* h,
-            uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps, hipStream_t st) {
+            uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps, int ceil, hipStream_t st) {
   const int64_t pitch = mx_pitch(cols), wide = OUT ? pitch : cols;
   // `most` rows a launch: f(first row, rows, the arrays from the first row on)
   auto go = [&](int64_t most, auto&& f) {
@@ -441,14 +442,14 @@ int rms_out(const T* x, int64_t xs, const R* r, int64_t rs, const W* w, T* y, ui
   };
   if (wide > kLong)
     return go(most_groups(1024), [&](int64_t n, auto x, auto r, auto y, auto codes, auto scales, auto h, auto low, auto rstd) {
-      k_rms_long<T, R, W, OUT><<<(uint32_t)n, 1024, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd, cols, eps);
+      k_rms_long<T, R, W, OUT><<<(uint32_t)n, 1024, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd, cols, eps, ceil);
       return check_launch("k_rms_long");
     });
   return with_shape<true>(wide, [&](auto tpr, auto nc) {
     constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, B = TPR < 256 ? 256 : TPR, K = B / TPR;
     return go(most_groups(B) * K, [&](int64_t n, auto x, auto r, auto y, auto codes, auto scales, auto h, auto low, auto rstd) {
       k_rms<T, R, W, OUT, TPR, NC><<<(uint32_t)((n + K - 1) / K), B, 0, st>>>(x, xs, r, rs, w, y, codes, scales, h, low, rstd,
-                                                                              n, cols, eps);
+                                                                              n, cols, eps, ceil);
       return check_launch("k_rms");
     });
   });
@@ -456,11 +457,12 @@ int rms_out(const T* x, int64_t xs, const R* r, int64_t rs, const W* w, T* y, ui
 
 template <typename T, typename R, typename W>
 int rms(int out, const void* x, int64_t xs, const void* r, int64_t rs, const void* w, void* y, uint8_t* codes,
-        uint8_t* scales, void* h, uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps, hipStream_t st) {
+        uint8_t* scales, void* h, uint32_t* low, float* rstd, int64_t rows, int64_t cols, float eps, int ceil,
+        hipStream_t st) {
   auto go = [&](auto o) {
     return rms_out<T, R, W, decltype(o)::value>(static_cast<const T*>(x), xs, static_cast<const R*>(r), rs,
                                                 static_cast<const W*>(w), static_cast<T*>(y), codes, scales,
-                                                static_cast<R*>(h), low, rstd, rows, cols, eps, st);
+                                                static_cast<R*>(h), low, rstd, rows, cols, eps, ceil, st);
   };
   if (out == 0) return go(std::integral_constant<int, 0>{});
   if (out == 1 + kFp4) return go(std::integral_constant<int, 1 + kFp4>{});
@@ -526,6 +528,8 @@ extern "C" int a8_rms_norm(int dtype, int res_dtype, int w_dtype, int out_fmt, c
                            float eps, void* stream) {
   if (int e = check_types(dtype, res_dtype, w_dtype, "rms_norm: x must be fp32, bf16 or fp16, the residual and the "
                                                      "weight of that type or fp32")) return e;
+  const int ceil = out_fmt >= 0 && (out_fmt & A8_MX_CEIL) != 0;
+  if (ceil) out_fmt &= ~A8_MX_CEIL;
   if (out_fmt != A8_MX_NONE && out_fmt != A8_MXFP4 && out_fmt != A8_MXFP8)
     return set_error(A8_ERR_ARG, "rms_norm: unknown output format");
   if (rows < 0 || rows >= kLim || cols < 1 || cols >= kLim) return set_error(A8_ERR_SIZE, "rms_norm: rows or cols out of range");
@@ -536,7 +540,7 @@ extern "C" int a8_rms_norm(int dtype, int res_dtype, int w_dtype, int out_fmt, c
   if (out_fmt != A8_MX_NONE && !aligned16(codes)) return set_error(A8_ERR_ALIGN, "rms_norm: codes must be 16-byte aligned");
   return with_types(dtype, res_dtype, w_dtype, [&](auto t, auto r, auto w) {
     return rms<decltype(t), decltype(r), decltype(w)>(out_fmt + 1, x, x_stride, residual, r_stride, weight, y, codes, scales,
-                                                      h, h_low, rstd, rows, cols, eps, static_cast<hipStream_t>(stream));
+                                                      h, h_low, rstd, rows, cols, eps, ceil, static_cast<hipStream_t>(stream));
   });
 }
 

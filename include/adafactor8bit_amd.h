@@ -805,6 +805,7 @@ int a8_apollo_writeback(int dtype, int grad_native, int stochastic, void* param,
 #define A8_MX_NONE (-1)
 #define A8_MXFP4 0
 #define A8_MXFP8 1
+#define A8_MX_CEIL 0x100   /* OR'd into a8_rms_norm's out_fmt: scale_rule 1 */
 
 int64_t a8_mx_pitch(int64_t cols);
 
@@ -835,8 +836,8 @@ int a8_mx_matmul(int fmt_a, int fmt_b, int out_dtype, const uint8_t* a_codes, co
 
 /* h = x + residual (h = x without one; h, of the residual's type, is written only
  * with one), s = (mean(h^2) + eps)^-1/2 over each row, y = h s weight in x's type,
- * or with out_fmt A8_MXFP4 / A8_MXFP8 as an MX tensor (codes, scales; scale_rule 0,
- * nearest).  The sum h enters the norm before it is rounded to its type.  h_low
+ * or with out_fmt A8_MXFP4 / A8_MXFP8 as an MX tensor (codes, scales; nearest codes,
+ * scale_rule 0, or 1 with A8_MX_CEIL OR'd into out_fmt).  The sum h enters the norm before it is rounded to its type.  h_low
  * (optional, for a 16-bit residual type; else not written): rows * ((cols + 7) / 8) words, the next
  * four bits of h, for the backward pass.  rstd (optional): s per row.  residual and weight: x's type or fp32.  y and h are
  * contiguous; x and residual have rows x_stride / r_stride elements apart. */
