@@ -56,7 +56,8 @@ class Model(torch.nn.Module):
 
 
 class Server:
-    """The trained model with its projections laid out once: 4-bit blocks, the head in 8 bits."""
+    """The trained model with its projections laid out once: 4-bit blocks, the head in 8 bits; scales by the
+    rule that mx_linear trained with."""
 
     def __init__(self, model):
         with torch.no_grad():
@@ -71,10 +72,10 @@ class Server:
         """[sequences] x 2 -> [sequences, VOCAB]: one token of each sequence."""
         h, d = self.m.before[before], self.m.last[last]
         for i in range(BLOCKS):
-            y, h = rms_norm(d, self.m.gains[i], residual=h, out_fmt="mxfp8")
+            y, h = rms_norm(d, self.m.gains[i], residual=h, out_fmt="mxfp8", scale="ceil")
             a, b = mx_matmul(y, self.up[i], torch.float32).chunk(2, -1)
-            d = mx_matmul(mx_quantize(F.silu(a) * b, "mxfp8"), self.down[i], torch.float32)
-        y, h = rms_norm(d, self.m.gains[BLOCKS], residual=h, out_fmt="mxfp8")
+            d = mx_matmul(mx_quantize(F.silu(a) * b, "mxfp8", scale="ceil"), self.down[i], torch.float32)
+        y, h = rms_norm(d, self.m.gains[BLOCKS], residual=h, out_fmt="mxfp8", scale="ceil")
         return mx_matmul(y, self.head, torch.float32)
 
     def answer(self, start, length):

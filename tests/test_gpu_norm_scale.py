@@ -48,3 +48,20 @@ def test_refusals():
     n = nat.lib().a8_rms_norm
     for fmt in (2, 0x102, 0x200, -2, 0x100 - 0x200):
         assert n(0, 0, 0, fmt, 16, 1, None, 0, 16, 16, 16, 16, None, None, None, 1, 1, 1e-6, None) == -1
+
+
+def test_the_example_serves_what_it_trained():
+    """One rule in training and serving: a step of examples/mx_lm.py's server has the model's logits."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    try:
+        import mx_lm
+    finally:
+        sys.path.pop(0)
+    torch.manual_seed(3)
+    model = mx_lm.Model().cuda()
+    pairs = torch.randint(0, mx_lm.VOCAB, (16, 2)).cuda()
+    with torch.no_grad():
+        want = model(pairs)[:, 0]
+    assert torch.equal(mx_lm.Server(model).logits(pairs[:, 0], pairs[:, 1]), want)
