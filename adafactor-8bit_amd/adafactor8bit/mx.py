@@ -290,7 +290,8 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     product reads its operands in blocks along the summed dimension: the output from x and weight
     along k, x's gradient from dy and weight^T along n, the weight's gradient from dy^T and x^T along
     the rows.  For the backward pass only the transposed blocks are kept.  ``seed``: a whole number
-    rounds dy stochastically (pass another one each step); None rounds to nearest.  ``scale`` is the
+    rounds dy stochastically; None rounds to nearest.  Its random bits go by an element's place, so
+    pass another one in each step and in each layer: layers of one seed round alike.  ``scale`` is the
     rule of every operand; "ceil" saturates nothing, so that stochastic rounding has no bias.  The gradients
     have none themselves: ``create_graph`` is refused, and so are forward-mode derivatives.
 

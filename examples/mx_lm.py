@@ -45,14 +45,14 @@ class Model(torch.nn.Module):
         self.head = p(VOCAB, HIDDEN, scale=HIDDEN ** -0.5)
 
     def forward(self, tokens, seed=None):
-        """Logits of the token after each adjacent pair."""
+        """Logits of the token after each adjacent pair.  ``seed``: each projection takes one of its own from it on."""
         h, d = self.before[tokens[..., :-1]], self.last[tokens[..., 1:]]
         for i in range(BLOCKS):
             y, h = rms_norm(d, self.gains[i], residual=h)
             a, b = mx_linear(y, self.up[i], seed=None if seed is None else 2 * i + seed).chunk(2, -1)
             d = mx_linear(F.silu(a) * b, self.down[i], seed=None if seed is None else 2 * i + 1 + seed)
         y, h = rms_norm(d, self.gains[BLOCKS], residual=h)
-        return mx_linear(y, self.head, weight_fmt="mxfp8", seed=seed)
+        return mx_linear(y, self.head, weight_fmt="mxfp8", seed=None if seed is None else 2 * BLOCKS + seed)
 
 
 class Server:
