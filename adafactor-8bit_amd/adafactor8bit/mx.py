@@ -12,6 +12,7 @@ rule, under which the block's largest elements may saturate) or the next power o
 would saturate (``scale="ceil"``).  A block that holds a NaN or an infinity reads as NaN.
 """
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -30,6 +31,16 @@ def _code(table, key, what):
         return table[key]
     except (KeyError, TypeError):
         raise ValueError(f"adafactor8bit: {what} must be one of {', '.join(map(str, table))}, got {key!r}") from None
+
+
+def _seed(seed):
+    """None, or the whole number's low 64 bits."""
+    if seed is None:
+        return None
+    try:
+        return operator.index(seed) & _MASK64
+    except TypeError:
+        raise TypeError(f"adafactor8bit: seed must be None or a whole number, got {seed!r}") from None
 
 
 def _pitch(cols):   # no shifts or masks here and in _bytes: torch.compile's symbolic sizes have none
@@ -179,7 +190,7 @@ def _quantize(x, fmt, f, along, down, rule, seed):
     d = _new(cols, rows, fmt, f, dev) if down else None
     _launch("a8_mx_quantize", x.get_device(), _DTYPE[x.dtype], f, rule, seed is not None, x.data_ptr(), rows, cols,
             x.stride(0) if rows > 1 and cols else cols, *(a._addresses()[:2] if along else (None, None)),
-            *(d._addresses()[:2] if down else (None, None)), 0 if seed is None else seed & _MASK64)
+            *(d._addresses()[:2] if down else (None, None)), seed or 0)
     return a, d
 
 
@@ -193,7 +204,7 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
     draws; the same seed, the same codes).  An MX tensor has no gradient: an x that requires one is refused
     where gradients are recorded.
     """
-    f, rule = _code(_FMT, fmt, "fmt"), _code(_RULE, scale, "scale")
+    f, rule, seed = _code(_FMT, fmt, "fmt"), _code(_RULE, scale, "scale"), _seed(seed)
     if x.dim() < 1:
         raise ValueError("adafactor8bit: mx_quantize takes a tensor of at least one dimension")
     if x.dtype not in _DTYPE:
@@ -300,7 +311,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     """
     fmts = ((act_fmt, _code(_FMT, act_fmt, "act_fmt")), (weight_fmt, _code(_FMT, weight_fmt, "weight_fmt")),
             (grad_fmt, _code(_FMT, grad_fmt, "grad_fmt")))
-    rule = _code(_RULE, scale, "scale")
+    rule, seed = _code(_RULE, scale, "scale"), _seed(seed)
     k = weight.shape[-1]
     if x.dim() < 1 or x.shape[-1] != k or len(weight.shape) != 2:
         raise ValueError(f"adafactor8bit: mx_linear of x {tuple(x.shape)} and weight {tuple(weight.shape)}")
