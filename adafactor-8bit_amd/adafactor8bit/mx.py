@@ -60,8 +60,10 @@ class MXTensor:
 
     def __init__(self, codes, scales, cols, fmt):
         f = _code(_FMT, fmt, "fmt")
+        if cols < 0:
+            raise ValueError(f"adafactor8bit: an MX tensor of {cols} columns")
         p = _pitch(cols)
-        rows = codes.shape[0]
+        rows = codes.shape[0] if codes.dim() else 0
         if codes.shape != (rows, p if f else p // 2) or scales.shape != (rows, p // 32):
             raise ValueError(f"adafactor8bit: a {fmt} tensor of {cols} columns has codes [rows, {p if f else p // 2}] and "
                              f"scales [rows, {p // 32}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
@@ -144,6 +146,11 @@ def no_tangents(what, *tensors):
                 raise RuntimeError(f"adafactor8bit: {what} has no forward-mode derivative, got a dual tensor")
 
 
+def _mx(t, what):
+    if not isinstance(t, MXTensor):
+        raise TypeError(f"adafactor8bit: {what} takes an MXTensor, got {type(t).__name__}")
+
+
 def _not_on_gpu(t, what):
     return RuntimeError(f"adafactor8bit: {what} runs on the GPU only, got an MX tensor on {t.keep[0].device} and {t.keep[-1].device}")
 
@@ -221,6 +228,7 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
 
 def mx_dequantize(t, dtype=torch.bfloat16):
     """The values of an MX tensor as a contiguous [rows, cols] matrix."""
+    _mx(t, "mx_dequantize")
     if dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_dequantize writes fp32, bf16 or fp16, got {dtype}")
     cp, sp, i = t._addresses()
@@ -249,6 +257,8 @@ def mx_matmul(a, b, out_dtype=torch.bfloat16):
     pairing of the formats, accumulated in fp32 and rounded once to ``out_dtype``.  (Where a side is
     in 8 bits the matrix cores cut the 64 products they add at a time at 2^-13 of the largest one's
     binade, about 1.5e-5 of a result's size for two 8-bit sides; products of 4-bit sides are exact.)"""
+    _mx(a, "mx_matmul")
+    _mx(b, "mx_matmul")
     _code(_DTYPE, out_dtype, "out_dtype")
     if b.cols != a.cols:
         raise ValueError(f"adafactor8bit: mx_matmul of {a.cols} and {b.cols} columns")
@@ -312,8 +322,7 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     fmts = ((act_fmt, _code(_FMT, act_fmt, "act_fmt")), (weight_fmt, _code(_FMT, weight_fmt, "weight_fmt")),
             (grad_fmt, _code(_FMT, grad_fmt, "grad_fmt")))
     rule, seed = _code(_RULE, scale, "scale"), _seed(seed)
-    k = weight.shape[-1]
-    if x.dim() < 1 or x.shape[-1] != k or len(weight.shape) != 2:
+    if x.dim() < 1 or len(weight.shape) != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"adafactor8bit: mx_linear of x {tuple(x.shape)} and weight {tuple(weight.shape)}")
     if x.dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16, got {x.dtype}")
