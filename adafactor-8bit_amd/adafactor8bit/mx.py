@@ -179,7 +179,9 @@ def _launch(name, i, *args):
 
 
 def _rows(x):
-    """x as a matrix of its last dimension's rows, whose elements are adjacent (a copy where they are not)."""
+    """x as a matrix of its last dimension's rows, whose elements are adjacent (a copy where they are not, or
+    where their sign is still to be applied)."""
+    x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if x.is_contiguous():

@@ -45,8 +45,8 @@ class _RmsNorm(torch.autograd.Function):
             return (None, None, None, None) if dh is None else (dh.to(ctx.dtype), dh, None, None)
         h, low, weight, rstd = ctx.saved_tensors
         rows, cols = h.shape
-        dy = dy.contiguous()
-        dh = None if dh is None else dh.contiguous()
+        dy = dy.resolve_neg().contiguous()
+        dh = None if dh is None else dh.resolve_neg().contiguous()
         dx = torch.empty_like(dy)
         dr = torch.empty_like(h) if ctx.residual and h.dtype != ctx.dtype else None
         dw = ws = None
@@ -101,7 +101,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None, scale="floor"):
         raise ValueError("adafactor8bit: rms_norm's output in MX blocks has no gradient; call it under torch.no_grad()")
     x2 = _rows(x)
     r2 = None if residual is None else _rows(residual)
-    w = weight.contiguous()
+    w = weight.resolve_neg().contiguous()
     if grad:
         out = _RmsNorm.apply(x2, r2, w, eps)
         y, h = out if r2 is not None else (out, None)

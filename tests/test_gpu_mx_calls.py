@@ -143,3 +143,28 @@ def test_compiled_programs_call_the_operators(rows):
             y, z = c(x), f(x)
             assert torch.equal(y, z)
             assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.autograd.grad(z, x, torch.ones_like(z))[0])
+
+
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate is a view with the sign still to be applied."""
+    re, im = _r(6, 1, 1), _r(6, 1, 2)
+    v = torch.complex(re, im).conj().imag
+    assert v.is_neg() and torch.equal(v, -im)
+    assert torch.equal(a8.mx_dequantize(a8.mx_quantize(v), torch.float32), a8.mx_dequantize(a8.mx_quantize(-im), torch.float32))
+    one = torch.ones(1, device="cuda")
+    assert torch.equal(a8.rms_norm(v, one), a8.rms_norm(-im, one))
+    assert torch.equal(a8.mx_linear(v, one[None]), a8.mx_linear(-im, one[None]))
+    x, g, w, dy = _r(5, 40, 3), _r(1, 40, 4)[0], _r(7, 40, 5), _r(5, 40, 6)
+    neg = torch._neg_view
+    assert torch.equal(a8.rms_norm(neg(x), neg(g), residual=neg(dy))[0], a8.rms_norm(-x, -g, residual=-dy)[0])
+    assert torch.equal(a8.mx_linear(neg(x), neg(w)), a8.mx_linear(-x, -w))
+    xr, gr, wr = (t.clone().requires_grad_() for t in (x, g, w))
+    y, h = a8.rms_norm(xr, gr, residual=xr)
+    for grads in ((neg(dy), neg(x)), (-dy, -x)):
+        got = torch.autograd.grad((y, h), (xr, gr), grads, retain_graph=True)
+        if grads[0].is_neg():
+            want = got
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, dz = a8.mx_linear(xr, wr), _r(5, 7, 7)
+    a, b = (torch.autograd.grad(y, (xr, wr), d, retain_graph=True) for d in (neg(dz), -dz))
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
