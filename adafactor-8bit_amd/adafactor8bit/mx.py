@@ -139,11 +139,11 @@ def _on_gpu(x, what):
 
 
 def no_tangents(what, *tensors):
-    """A launch that autograd does not see carries no tangent on: its result would read as a constant."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"adafactor8bit: {what} has no forward-mode derivative, got a dual tensor")
+    """A launch that autograd does not see carries no tangent on: its result would read as a constant.  (Called
+    where a dual level is entered, forward_ad._current_level >= 0.)"""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"adafactor8bit: {what} has no forward-mode derivative, got a dual tensor")
 
 
 def _mx(t, what):
@@ -181,7 +181,8 @@ def _launch(name, i, *args):
 def _rows(x):
     """x as a matrix of its last dimension's rows, whose elements are adjacent (a copy where they are not, or
     where their sign is still to be applied)."""
-    x = x.resolve_neg()
+    if x.is_neg():
+        x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if x.is_contiguous():
@@ -219,7 +220,8 @@ def mx_quantize(x, fmt="mxfp8", axis=1, scale="floor", seed=None):
     if x.dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_quantize takes fp32, bf16 or fp16, got {x.dtype}")
     _on_gpu(x, "mx_quantize")
-    no_tangents("mx_quantize", x)
+    if forward_ad._current_level >= 0:
+        no_tangents("mx_quantize", x)
     if axis not in (0, 1, "both"):
         raise ValueError(f"adafactor8bit: axis must be 0, 1 or 'both', got {axis!r}")
     if x.requires_grad and torch.is_grad_enabled():
@@ -275,7 +277,8 @@ def first_order(name, gradients):
     def backward(ctx, *dy):
         if torch.is_grad_enabled():
             raise RuntimeError(f"adafactor8bit: {name} cannot be differentiated twice; call without create_graph")
-        no_tangents(f"{name}'s backward pass", *dy)
+        if forward_ad._current_level >= 0:
+            no_tangents(f"{name}'s backward pass", *dy)
         return plain(ctx, *dy)
 
     return staticmethod(backward)
@@ -329,7 +332,8 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     if x.dtype not in _DTYPE:
         raise TypeError(f"adafactor8bit: mx_linear takes fp32, bf16 or fp16, got {x.dtype}")
     _on_gpu(x, "mx_linear")
-    no_tangents("mx_linear", x, None if isinstance(weight, MXTensor) else weight)
+    if forward_ad._current_level >= 0:
+        no_tangents("mx_linear", x, None if isinstance(weight, MXTensor) else weight)
     if weight.device != x.device:
         raise ValueError("adafactor8bit: mx_linear's operands are on one device")
     blocks = isinstance(weight, MXTensor)

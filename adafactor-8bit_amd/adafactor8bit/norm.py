@@ -4,11 +4,16 @@ An addition of this build: the norm in front of every projection of the models w
 optimizer holds, writing the 8-bit activations that ``mx_matmul`` reads.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .mx import _DTYPE, _FMT, _RULE, _code, _launch, _new, _on_gpu, _rows, first_order, no_tangents
 
 _DENSE = torch.contiguous_format
+
+
+def _dense(t):
+    return t if t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
 
 
 def _forward(x, residual, weight, eps, fmt, keep, rule=0):
@@ -45,8 +50,8 @@ class _RmsNorm(torch.autograd.Function):
             return (None, None, None, None) if dh is None else (dh.to(ctx.dtype), dh, None, None)
         h, low, weight, rstd = ctx.saved_tensors
         rows, cols = h.shape
-        dy = dy.resolve_neg().contiguous()
-        dh = None if dh is None else dh.resolve_neg().contiguous()
+        dy = _dense(dy)
+        dh = None if dh is None else _dense(dh)
         dx = torch.empty_like(dy)
         dr = torch.empty_like(h) if ctx.residual and h.dtype != ctx.dtype else None
         dw = ws = None
@@ -94,14 +99,15 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out_fmt=None, scale="floor"):
             raise ValueError(f"adafactor8bit: rms_norm of x {tuple(shape)} with residual {tuple(residual.shape)}")
         if residual.dtype != dtype and residual.dtype != torch.float32:
             raise TypeError(f"adafactor8bit: rms_norm's residual is {dtype} or fp32, got {residual.dtype}")
-    no_tangents("rms_norm", x, weight, residual)
+    if forward_ad._current_level >= 0:
+        no_tangents("rms_norm", x, weight, residual)
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                         or (residual is not None and residual.requires_grad))
     if grad and out_fmt is not None:
         raise ValueError("adafactor8bit: rms_norm's output in MX blocks has no gradient; call it under torch.no_grad()")
     x2 = _rows(x)
     r2 = None if residual is None else _rows(residual)
-    w = weight.resolve_neg().contiguous()
+    w = _dense(weight)
     if grad:
         out = _RmsNorm.apply(x2, r2, w, eps)
         y, h = out if r2 is not None else (out, None)
