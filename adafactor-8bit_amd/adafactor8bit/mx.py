@@ -319,7 +319,8 @@ def mx_linear(x, weight, act_fmt="mxfp8", weight_fmt="mxfp4", grad_fmt="mxfp8", 
     rounds dy stochastically; None rounds to nearest.  Its random bits go by an element's place, so
     pass another one in each step and in each layer: layers of one seed round alike.  ``scale`` is the
     rule of every operand; "ceil" saturates nothing, so that stochastic rounding has no bias.  The gradients
-    have none themselves: ``create_graph`` is refused, and so are forward-mode derivatives.
+    have none themselves: ``create_graph`` is refused, and so are forward-mode derivatives. Products with an
+    8-bit side have the precision that mx_matmul names, gradients of fp32 tensors among them.
 
     ``weight`` may be an MXTensor laid out once (serving): x is then quantised and multiplied, without
     gradients.

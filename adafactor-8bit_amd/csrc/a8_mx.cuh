@@ -159,8 +159,8 @@ __device__ __forceinline__ void mx_sr4(float* t, uint64_t r) {
   }
 }
 
-// Four consecutive elements' 16 random bits each: one output of SplitMix64, whose
-// counter is sr_base(seed, orientation) + (element index / 4).
+// Four consecutive elements' 16 random bits each: one output of SplitMix64, whose counter is base +
+// (element index / 4), base = seed * 0x9E3779B97F4A7C15, for the transpose + 0xD1B54A32D192ED03.
 __device__ __forceinline__ uint64_t mx_random(uint64_t base, uint64_t word) {
   uint64_t z = base + word + 0x9E3779B97F4A7C15ULL;
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
